@@ -50,15 +50,23 @@ class _NormAddNormFn(Function):
             return (None,) * 8
         dh = None if dh is None else _packed(dh)
         ds = None if ds is None else _packed(ds)
-        bufs, rets, add, used = [None] * 3, [None] * 3, 0, []
+        bufs, rets, add, used, again = [None] * 3, [None] * 3, 0, [], []
         for i, (w, need) in enumerate(((w1, ctx.needs_input_grad[2]), (gate, ctx.needs_input_grad[4]),
                                        (w2, ctx.needs_input_grad[3]))):
             if w is None or not need:
                 continue
-            bufs[i], more, rets[i] = _target(w)
+            buf, more, rets[i] = _target(w)
+            if any(b is not None and b.data_ptr() == buf.data_ptr() for b in bufs):
+                # one parameter in two roles: the kernel writes its targets independently of each other
+                again.append((buf, torch.empty_like(buf, dtype=torch.float32)))
+                bufs[i] = again[-1][1]
+                continue
+            bufs[i] = buf
             add |= int(more) << i
             used.append(w)
         dx, dres = lib().block_norm_bwd(dh, ds, x, res, w1, w2, gate, r1, r2, alpha, offset, *bufs, add)
+        for buf, part in again:
+            buf.add_(part)
         for w in used:
             if getattr(w, "main_grad", None) is not None:
                 w.grad_added = True
