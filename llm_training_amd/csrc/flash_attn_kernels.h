@@ -248,7 +248,8 @@ struct AttnArgs {
 //             instead of a tanh; its derivative is 4 (r - r^2), whose 4 goes into the gradients' final scale;
 //   kModBias  one subtraction and one FMA per score (|.| is an operand modifier);
 //   kModPre   kernels without either that read a.pend. (Every MOD kernel reads it: a prefix only changes the index
-//             ranges of the masks and the tiles walked, nothing per score.)
+//             ranges of the masks and the tiles walked, nothing per score.) As the kernels on plain scores they take
+//             maxima and masks of raw products, so a scale <= 0 runs the kernels with a bias, of slope 0.
 // MOD = 0 leaves all of it out of the kernels on plain scores.
 //
 // The MOD forward divides O by the sum of the bf16 probabilities that the product uses (the LSE keeps the sum of the
@@ -1442,8 +1443,12 @@ __global__ __launch_bounds__(256, 1) void fa_bwd_dkdv5_kernel(AttnArgs a, const 
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           if (!in_range(rg, 8 * (i >> 2) + (i & 3))) {
-            sc[i] = -INFINITY;
-            if constexpr (MOD & kModCap) lq[i] = -INFINITY;  // (a capped -inf is finite)
+            if constexpr (MOD & (kModCap | kModBias)) {  // (a capped -inf is finite, and a scale <= 0 turns its sign)
+              sc[i] = 0.f;
+              lq[i] = -INFINITY;
+            } else {
+              sc[i] = -INFINITY;
+            }
           }
         return;
       }
@@ -2207,17 +2212,18 @@ __global__ __launch_bounds__(NW * 64, 2) void fa_bwd_dq3_kernel(AttnArgs a) {
           for (int i = 0; i < 16; ++i) st[i] = fmaf(-st[i], st[i], st[i]) * dpt[i];
         } else if constexpr (MOD & kModBias) {
           const float d0 = (float)(qrow - n0 - 32 * tt - 4 * hh), base = score_base<MOD>(a, -lse2);
-          if (need_mask) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float rr;
+            st[i] = mod_score<MOD>(a, st[i], sl2, nslope, d0 - (float)(8 * (i >> 2) + (i & 3)), base, rr);
+          }
+          if (need_mask) {  // (the scores, not the products: a scale <= 0 would turn a product's -inf)
             const IdxRange rg = idx_range(klo, khi, n0 + 32 * tt + 4 * hh);
 #pragma unroll
             for (int i = 0; i < 16; ++i) st[i] = in_range(rg, 8 * (i >> 2) + (i & 3)) ? st[i] : -INFINITY;
           }
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float rr;
-            const float x = mod_score<MOD>(a, st[i], sl2, nslope, d0 - (float)(8 * (i >> 2) + (i & 3)), base, rr);
-            st[i] = fexp2(x) * (dpt[i] - dlt);
-          }
+          for (int i = 0; i < 16; ++i) st[i] = fexp2(st[i]) * (dpt[i] - dlt);
         } else if (need_mask && !OM) {
           const IdxRange rg = idx_range(klo, khi, n0 + 32 * tt + 4 * hh);
 #pragma unroll
@@ -2323,7 +2329,7 @@ __global__ __launch_bounds__(NW * 64, 2) void fa_bwd_dq3_kernel(AttnArgs a) {
 // side), with `mod` as mod_of() gives it.
 inline int mod_of(const AttnArgs& a) {
   const int m = (a.cap_z > 0.f ? kModCap : 0) | (a.slopes || a.cap_z > kFixCap * kLog2e ? kModBias : 0);
-  return m ? m : a.pend ? kModPre : 0;
+  return m || !a.pend ? m : a.scale > 0.f ? kModPre : kModBias;
 }
 hipError_t launch_mod_fwd(const AttnArgs& a, int D, int mod, unsigned grid, hipStream_t stream);
 hipError_t launch_mod_dq(const AttnArgs& a, int D, int mod, unsigned grid, hipStream_t stream);

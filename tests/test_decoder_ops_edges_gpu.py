@@ -3,6 +3,8 @@ import pytest
 import torch
 
 from llm_training_amd import ops
+from test_attention_mod_gpu import MODS
+from test_attention_mod_gpu import run as attention
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -34,3 +36,12 @@ def test_norm_add_norm_one_parameter_in_two_roles(roles, added):
     want = want + (3.0 if added else 0.0)
     assert ((w.main_grad.double() - want).abs() <= 2.0 ** -16 * size).all()
     assert w.grad_added and w.grad is None
+
+
+@pytest.mark.parametrize("mod", list(MODS))
+@pytest.mark.parametrize("scale", [-0.125, 0.0])
+@pytest.mark.parametrize("kw", [dict(), dict(ndocs=3), dict(window=40)])
+def test_modified_scores_with_a_scale_of_zero_or_below(mod, scale, kw):
+    """Masked scores stay masked whatever the sign that a product of -inf would take."""
+    got = attention(2, 200, 4, 2, 64, scale=scale, **kw, **MODS[mod])
+    assert all(t.isfinite().all() for t in got)
