@@ -258,14 +258,18 @@ struct AttnArgs {
 // window) loses dS to the cancellation: relative errors of dQ over rows of 2 / 8 / 256 keys 17 / 6 / 4.6e-3 without,
 // 2.6e-3 with both, whatever the length. It costs the second store and half an instruction per probability, so a
 // forward without a backward to follow (no a.olo, template argument LO false) divides by the sum of the unrounded
-// ones, as plain attention does: 1 x 8192, 32 heads of 64, distance bias 410 -> 387 us. (Not under kModCap alone, whose
-// largest probability is not 1: a row of one key would not be that key's value.)
+// ones, as plain attention does: 1 x 8192, 32 heads of 64, distance bias 430 -> 405 us. (Not under kModCap alone, whose
+// rows may keep a reference below their maximum: a row of one key would not be that key's value.)
 constexpr int kModCap = 1, kModBias = 2, kModPre = 4;
 
-// Capped scores lie in [-cap_z, cap_z]: up to kFixCap the MOD = kModCap forward takes its probabilities against 0
-// instead of the running row maximum (2^+-87 at most: fp32 and bf16 hold them and their sums), which drops the maximum,
-// the rescaling and one subtraction per score. Larger caps run the kernels with a bias, of slope 0.
-constexpr float kFixCap = 60.f;
+// Capped scores lie in [-cap_z, cap_z]. Up to kCapMax the MOD = kModCap forward starts its running maximum at -cap_z and
+// subtracts it in the polynomial's last FMA, where it is free: a tile's scores are relative to the maximum before it and
+// are moved only where that grows by more than kThr. (Probabilities against 0 without a maximum, up to 2^87, took 350
+// instead of 360 us of 2 x 4096, 32 / 8 heads of 128, and 463 instead of 488 of 1 x 8192, 32 of 64, and overflowed with
+// values of V from 1e9 on. Skipping the maximum of tiles whose largest product bounds their scores gained nothing.) The
+// dQ kernel takes masked scores as 0, whose probability, 2^cap_z at most, has to be finite. Larger caps run the kernels
+// with a bias, of slope 0.
+constexpr float kCapMax = 60.f;
 
 // score_base() + the score in log2 units from the raw product x; rr: the tanh's derivative / 4
 template <int MOD>
@@ -288,9 +292,9 @@ __device__ __forceinline__ float mod_score(const AttnArgs& a, float x, float sl2
 // which take four instructions' time each, and two more. set_mod scales the coefficients to the raw product x. (Forward,
 // cap 50: 1 x 8192, 32 heads of 64 470 -> 443 us, 2 x 4096, 32 of 96 307 -> 287, 32 of 128 357 -> 353. The dQ kernel has
 // the tanh's derivative to take too and lost 2 % by it.)
-__device__ __forceinline__ float small_cap(const AttnArgs& a, float x) {
+__device__ __forceinline__ float small_cap(const AttnArgs& a, float x, float c) {  // (plus c)
   const float s = x * x;
-  return x * fmaf(s, fmaf(s, fmaf(s, a.cap_q3, a.cap_q2), a.cap_q1), a.cap_q0);
+  return fmaf(x, fmaf(s, fmaf(s, fmaf(s, a.cap_q3, a.cap_q2), a.cap_q1), a.cap_q0), c);
 }
 // whether all the wave's scores may take it
 __device__ __forceinline__ bool all_small(const AttnArgs& a, const f32v16& x) {
@@ -1724,8 +1728,8 @@ __global__ __launch_bounds__(NW * 64, 2) void fa_fwd3_kernel(AttnArgs a) {
   float m = -INFINITY, l = 0.f;  // running max in scaled log2 units
   float lb = 0.f;                // MOD: sum of the bf16 probabilities (l: of the unrounded ones)
   constexpr bool Z = (MOD & (kModCap | kModBias)) != 0;  // the scores are turned into log2 units first
-  constexpr bool FIX = MOD == kModCap;                   // probabilities against 0 (see kFixCap)
-  if constexpr (FIX) m = 0.f;
+  constexpr bool CAP = MOD == kModCap;                   // the running max goes into the scores' last FMA
+  if constexpr (CAP) m = -a.cap_z;                       // (no score lies below it)
   float sl2v = sl2;  // (a VGPR: an FMA reads one scalar register at most, the element's)
   if constexpr (MOD & kModBias) asm volatile("" : "+v"(sl2v));
   float belem[16];  // bias: score_base - nslope * (the element's offset in its half tile), uniform: scalar registers
@@ -1815,14 +1819,14 @@ __global__ __launch_bounds__(NW * 64, 2) void fa_fwd3_kernel(AttnArgs a) {
           for (int tt = 0; tt < 2; ++tt) {
             if (all_small(a, st[tt])) {
 #pragma unroll
-              for (int i = 0; i < 16; ++i) st[tt][i] = small_cap(a, st[tt][i]);
+              for (int i = 0; i < 16; ++i) st[tt][i] = small_cap(a, st[tt][i], -m);
               asm volatile("" : "+v"(st[tt]));
             } else {
-              const float base = score_base<MOD>(a, 0.f);
+              const float base = score_base<MOD>(a, 0.f);  // (with -m in it the compiler holds 16 copies: spills)
 #pragma unroll
               for (int i = 0; i < 16; ++i) {
                 float rr;
-                st[tt][i] = mod_score<MOD>(a, st[tt][i], sl2, 0.f, 0.f, base, rr);
+                st[tt][i] = mod_score<MOD>(a, st[tt][i], sl2, 0.f, 0.f, base, rr) - m;
               }
               asm volatile("" : "+v"(st[tt]));
             }
@@ -1863,35 +1867,45 @@ __global__ __launch_bounds__(NW * 64, 2) void fa_fwd3_kernel(AttnArgs a) {
             }
           }
       }
-      if constexpr (!FIX) {
-        float mx0 = vmax3(st[0][0], st[0][1], st[0][2]), mx1 = vmax3(st[1][0], st[1][1], st[1][2]);
+      float mx0 = vmax3(st[0][0], st[0][1], st[0][2]), mx1 = vmax3(st[1][0], st[1][1], st[1][2]);
 #pragma unroll
-        for (int i = 3; i < 15; i += 2) {
-          mx0 = vmax3(mx0, st[0][i], st[0][i + 1]);
-          mx1 = vmax3(mx1, st[1][i], st[1][i + 1]);
-        }
-        float smax = vmax3(mx0, st[0][15], vmax3(mx1, st[1][15], mx1));
-        if constexpr (MOD & kModBias)  // (here: the two half-waves' parts differ)
-          smax = fmaxf(fmaxf(mx0, st[0][15]) + rowb[0], fmaxf(mx1, st[1][15]) + rowb[1]);
-        if constexpr (RS == 2) {  // the two half-waves' maxima through one permlane32 swap (no LDS round trip)
-          const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(smax), __float_as_uint(smax), false, false);
-          smax = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
-          if constexpr (!Z) smax *= sl2;
+      for (int i = 3; i < 15; i += 2) {
+        mx0 = vmax3(mx0, st[0][i], st[0][i + 1]);
+        mx1 = vmax3(mx1, st[1][i], st[1][i + 1]);
+      }
+      float smax = vmax3(mx0, st[0][15], vmax3(mx1, st[1][15], mx1));
+      if constexpr (MOD & kModBias)  // (here: the two half-waves' parts differ)
+        smax = fmaxf(fmaxf(mx0, st[0][15]) + rowb[0], fmaxf(mx1, st[1][15]) + rowb[1]);
+      if constexpr (RS == 2) {  // the two half-waves' maxima through one permlane32 swap (no LDS round trip)
+        const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(smax), __float_as_uint(smax), false, false);
+        smax = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+        if constexpr (!Z) smax *= sl2;
+      } else {
+        smax = fmaxf(smax, __shfl_xor(smax, 32, 64)) * sl2;
+      }
+      // deferred rescale: keep the running max unless some row grew by more than kThr
+      if (__any(smax > (CAP ? kThr : m + kThr))) {
+        float alpha;
+        if constexpr (CAP) {  // (the scores are relative to m, which moves by `up`)
+          const float up = fmaxf(smax, 0.f);
+          alpha = fexp2(-up);
+          m += up;
+#pragma unroll
+          for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) st[tt][i] -= up;
+          asm volatile("" : "+v"(st[0]), "+v"(st[1]));
         } else {
-          smax = fmaxf(smax, __shfl_xor(smax, 32, 64)) * sl2;
-        }
-        // deferred rescale: keep the running max unless some row grew by more than kThr
-        if (__any(smax > m + kThr)) {
           const float mnew = fmaxf(m, smax);
-          const float alpha = (mnew == -INFINITY) ? 1.f : fexp2(m - mnew);
+          alpha = (mnew == -INFINITY) ? 1.f : fexp2(m - mnew);
           m = mnew;
-          l *= alpha;
-          if constexpr (MOD && LO) lb *= alpha;
-#pragma unroll
-          for (int dt = 0; dt < NDT; ++dt)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) ot[dt][i] *= alpha;
         }
+        l *= alpha;
+        if constexpr (MOD && LO) lb *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) ot[dt][i] *= alpha;
       }
       const float nm = (m == -INFINITY) ? 0.f : -m;
       if constexpr (MOD & kModBias) {
@@ -1907,8 +1921,8 @@ __global__ __launch_bounds__(NW * 64, 2) void fa_fwd3_kernel(AttnArgs a) {
             // exp pair + row-sum adds in one asm block: each add sits one instruction behind the exp it reads
             // (the trans-use wait state, by placement instead of an s_nop), and hipcc cannot pair the adds
             // into v_pk_add_f32
-            const float x0 = FIX ? st[tt][i] : Z ? st[tt][i] + rowb[tt] : fmaf(st[tt][i], sl2, nm);
-            const float x1 = FIX ? st[tt][i + 1] : Z ? st[tt][i + 1] + rowb[tt] : fmaf(st[tt][i + 1], sl2, nm);
+            const float x0 = CAP ? st[tt][i] : Z ? st[tt][i] + rowb[tt] : fmaf(st[tt][i], sl2, nm);
+            const float x1 = CAP ? st[tt][i + 1] : Z ? st[tt][i + 1] + rowb[tt] : fmaf(st[tt][i + 1], sl2, nm);
             float e0, e1;
             asm("v_exp_f32 %0, %4\n\tv_exp_f32 %1, %5\n\tv_add_f32 %2, %2, %0\n\tv_add_f32 %3, %3, %1"
                 : "=&v"(e0), "=&v"(e1), "+v"(rs0), "+v"(rs1)
@@ -2328,7 +2342,7 @@ __global__ __launch_bounds__(NW * 64, 2) void fa_bwd_dq3_kernel(AttnArgs a) {
 // The launches of the MOD kernels (flash_attn_mod_fwd.hip / _dq.hip / _dkdv.hip, a file each: they compile side by
 // side), with `mod` as mod_of() gives it.
 inline int mod_of(const AttnArgs& a) {
-  const int m = (a.cap_z > 0.f ? kModCap : 0) | (a.slopes || a.cap_z > kFixCap * kLog2e ? kModBias : 0);
+  const int m = (a.cap_z > 0.f ? kModCap : 0) | (a.slopes || a.cap_z > kCapMax * kLog2e ? kModBias : 0);
   return m || !a.pend ? m : a.scale > 0.f ? kModPre : kModBias;
 }
 hipError_t launch_mod_fwd(const AttnArgs& a, int D, int mod, unsigned grid, hipStream_t stream);

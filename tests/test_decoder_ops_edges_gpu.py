@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from llm_training_amd import ops
-from test_attention_mod_gpu import MODS
+from test_attention_mod_gpu import MODS, compare, oracle
 from test_attention_mod_gpu import run as attention
 
 pytestmark = pytest.mark.gpu
@@ -45,3 +45,36 @@ def test_modified_scores_with_a_scale_of_zero_or_below(mod, scale, kw):
     """Masked scores stay masked whatever the sign that a product of -inf would take."""
     got = attention(2, 200, 4, 2, 64, scale=scale, **kw, **MODS[mod])
     assert all(t.isfinite().all() for t in got)
+
+
+@pytest.mark.parametrize("D", [64, 96, 128])
+@pytest.mark.parametrize("softcap", [60.0, 50.0, 100.0])
+@pytest.mark.parametrize("size", [1e-30, 1e10, 1e30])
+def test_capped_scores_at_both_ends_and_values_of_any_size(D, softcap, size):
+    """Rows whose scores are saturated at the cap, at its negative, and at both: the probabilities are taken against the
+    row's maximum, so neither they nor their products with V leave fp32's range. dO is scaled so that dP stays of the
+    order of 1."""
+    torch.manual_seed(5)
+    S = 700
+    end = torch.tensor([1.0, -1.0, 0.0], device=DEV)[torch.arange(S, device=DEV) % 3]  # of the query's scores
+    mix = torch.where(torch.rand(S, device=DEV) < 0.5, 1.0, -1.0)                      # of the key
+    q, k = (torch.randn(1, S, 2, D, device=DEV) for _ in range(2))
+    q[..., 0], q[..., 1] = 400.0 * end[None, :, None], 400.0 * (1 - end.abs())[None, :, None]
+    k[..., 0], k[..., 1] = 40.0, 40.0 * mix[None, :, None]
+    v = torch.randn(1, S, 2, D, device=DEV) * size
+    q, k, v = (t.bfloat16().requires_grad_(True) for t in (q, k, v))
+    do = (torch.randn(1, S, 2, D, device=DEV) / size).bfloat16()
+    o = ops.flash_attention(q, k, v, softcap=softcap)
+    got = [o, *torch.autograd.grad(o, (q, k, v), do)]
+    with torch.no_grad():
+        want, lim = oracle(q, k, v, do, True, None, -1, D ** -0.5, softcap, None, None)
+        # The oracle's 1 - tanh^2 is 0 where the derivative is below 2^-52 (4e-24 here), and with it the bound's share of
+        # delta's and dP's errors, p dx (e_delta + 2^-11 mag). Up to 2^-52 of that share is added back: e_delta <=
+        # 2^-8 (max dP + max delta) <= 2^-8 mag, so 2^-52 (2^-8 + 2^-11) mag a score, and p sums to 1 over a row's keys.
+        mag = 2 * (do.double().abs().sum(-1).max() * v.double().abs().max())
+        share = D ** -0.5 * 2.0 ** -52 * (2.0 ** -8 + 2.0 ** -11) * mag
+        lim[1] += share * k.double().abs().max()
+        lim[2] += share * S * q.double().abs().max()
+        compare(got, want, lim)
+        plain = ops.flash_attention(q, k, v, softcap=softcap)
+    assert plain.isfinite().all() and torch.equal(o == 0, plain == 0)
