@@ -1158,7 +1158,7 @@ __device__ __forceinline__ void dma_tile9(const Rsrc& k, const Rsrc& v, const Rs
       : "=&s"(keep)
       : "s"(l0), "s"(img), "v"(vk[0]), "v"(vk[1]), "v"(vk[2]), "v"(vk[3]), "v"(vv[0]), "v"(vv[1]), "v"(vv[2]),
         "v"(vv[3]), "v"(vs), "s"(k.w), "s"(v.w), "s"(sg.w), "s"(__builtin_amdgcn_readfirstlane(lds_addr(lseg)))
-      : "memory");
+      : "memory", "scc");  // (the additions set it)
 }
 // the same with the descriptor forced to SGPRs (a kernel under SGPR pressure may keep it in VGPRs,
 // which the asm's "s" operand does not accept)
