@@ -179,6 +179,8 @@ constexpr int64_t kCustomStep = 64;
 bool is_custom(hipblasLtHandle_t h, hipblasLtMatmulAlgo_t& algo) {
   return hipblaslt_ext::getKernelNameFromAlgo(h, algo).rfind("Custom_", 0) == 0;
 }
+// The library's own split-K hands its steps out in whole ones: below two steps a split some split has a single one.
+bool splits_to_one_step(int64_t k, int gsu) { return k < 2 * kCustomStep * gsu; }
 
 // C (m x n, column-major) = op(A) . op(B) (+ C when accumulate); batch > 1: split-K into `batch` fp32 slabs
 // of C (C is then [batch, n, m] fp32 with ldc = m, k divisible by batch)
@@ -256,6 +258,7 @@ void gemm_lt_impl(const at::Tensor& A, const at::Tensor& B, at::Tensor C, bool t
     const bool gsu_try = !kGsu.empty() && batch == 1 && ((m + 255) / 256) * ((n + 255) / 256) < kGsuMaxTiles;
     if (pre != s.preset.end() && pre->second.first < got) {
       best = Choice{res[pre->second.first].algo, pre->second.first, 0.f, pre->second.second};
+      if (splits_to_one_step(k, best.gsu) && is_custom(h, best.algo)) best.gsu = 0;
     } else if ((s.tune || (!streamk && kTimeNoSk) || gsu_try) && (got > 1 || gsu_try)) {
       // time every candidate on the live operands; the output goes to a scratch tensor so an
       // accumulating call (beta = 1) is not disturbed
@@ -290,6 +293,7 @@ void gemm_lt_impl(const at::Tensor& A, const at::Tensor& B, at::Tensor C, bool t
       for (int i : ok) {
         if (!gsu_try) break;
         for (int gs : kGsu) {  // the same solution with the library's own split-K
+          if (splits_to_one_step(k, gs) && is_custom(h, res[i].algo)) continue;
           hipblaslt_ext::Gemm eg(h, d.op, &alpha, A.data_ptr(), d.a, B.data_ptr(), d.b, &beta, scratch.data_ptr(), d.c,
                                  scratch.data_ptr(), d.c);
           hipblaslt_ext::GemmTuning tun;
