@@ -44,6 +44,27 @@ def _dense_mask(seg: torch.Tensor, S: int, dtype, window: int | None) -> torch.T
     return m.masked_fill(~vis[:, None], torch.finfo(dtype).min)
 
 
+class _BatchProduct(torch.autograd.Function):
+    """a @ b, or a @ b^T, over leading dimensions, every product's right operand contiguous, in the backward too: the
+    library's batched bf16 products have faulted on right operands that are transposed views."""
+
+    @staticmethod
+    @torch.amp.custom_fwd(device_type="cuda")
+    def forward(ctx, a, b, trans):
+        ctx.save_for_backward(a, b)
+        ctx.trans = trans
+        return torch.matmul(a, (b.transpose(-1, -2) if trans else b).contiguous())
+
+    @staticmethod
+    @torch.amp.custom_bwd(device_type="cuda")
+    def backward(ctx, g):
+        a, b = ctx.saved_tensors
+        if ctx.trans:
+            return torch.matmul(g, b.contiguous()), torch.matmul(g.transpose(-1, -2), a.contiguous()), None
+        return (torch.matmul(g, b.transpose(-1, -2).contiguous()),
+                torch.matmul(a.transpose(-1, -2), g.contiguous()), None)
+
+
 def hf_attention(module, query, key, value, attention_mask, scaling=None, dropout=0.0, sliding_window=None,
                  softcap=None, **kwargs):
     """transformers attention function: query [B, Hq, S, D], key/value [B, Hkv, S, D] ->
@@ -74,7 +95,7 @@ def hf_attention(module, query, key, value, attention_mask, scaling=None, dropou
         from transformers.integrations.sdpa_attention import repeat_kv
         n_rep = query.shape[1] // key.shape[1]
         k, v = repeat_kv(key, n_rep), repeat_kv(value, n_rep)
-        s = torch.matmul(query, k.transpose(2, 3).contiguous()) * (scaling if scaling is not None else D ** -0.5)
+        s = _BatchProduct.apply(query, k, True) * (scaling if scaling is not None else D ** -0.5)
         s = torch.tanh(s / softcap) * softcap
         S = query.shape[2]
         if attention_mask is None:
@@ -84,7 +105,7 @@ def hf_attention(module, query, key, value, attention_mask, scaling=None, dropou
             s = s + attention_mask
         p = torch.nn.functional.dropout(torch.softmax(s.float(), -1).to(query.dtype), dropout,
                                         training=module.training)
-        return torch.matmul(p, v).transpose(1, 2).contiguous(), None
+        return _BatchProduct.apply(p, v, False).transpose(1, 2).contiguous(), None
     return sdpa_attention_forward(module, query, key, value, attention_mask, scaling=scaling, dropout=dropout)
 
 

@@ -1,7 +1,11 @@
 """Calls of the decoder operators at the edge of what their documentation allows, as far as the host decides them."""
+from types import SimpleNamespace
+
 import torch
+from torch.utils._python_dispatch import TorchDispatchMode
 
 from llm_training_amd import ops
+from llm_training_amd.models.hf_causal_lm import hf_attention
 from llm_training_amd.ops import block_norm as bn
 from llm_training_amd.ops import reference as ref
 
@@ -47,3 +51,41 @@ def test_norm_add_norm_one_parameter_in_two_roles(monkeypatch):
             torch.autograd.backward(y, (dh, ds))
             assert torch.allclose(w.main_grad, plain + (3.0 if added else 0.0), atol=1e-5), (roles, added)
             assert w.grad_added and w.grad is None
+
+
+def _capped64(q, k, v, scale, cap, window=None):
+    """Causal capped attention of [B, H, S, D] in 64 bits, [B, S, H, D]."""
+    g = q.shape[1] // k.shape[1]
+    k, v = k.repeat_interleave(g, 1), v.repeat_interleave(g, 1)
+    i = torch.arange(q.shape[2])
+    s = cap * torch.tanh(q @ k.transpose(-1, -2) * scale / cap)
+    see = i[None] <= i[:, None]
+    if window is not None:
+        see &= i[:, None] - i[None] < window
+    return (torch.softmax(s.masked_fill(~see, float("-inf")), -1) @ v).transpose(1, 2)
+
+
+def test_dense_capped_attention_multiplies_by_contiguous_operands():
+    """The dense path of capped attention (here: a cap beyond the kernels' range): no product, forward or backward, has a
+    transposed view on its right, and the gradients are those of the formula."""
+    m = SimpleNamespace(is_causal=True, training=False)
+    seen = []
+
+    class Products(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            if func in (torch.ops.aten.bmm.default, torch.ops.aten.baddbmm.default):
+                seen.append(args[-1].is_contiguous())
+            return func(*args, **(kwargs or {}))
+
+    torch.manual_seed(0)
+    q = torch.randn(2, 7, 4, 6, dtype=torch.float64).transpose(1, 2).requires_grad_(True)
+    k, v = (torch.randn(2, 7, 2, 6, dtype=torch.float64).transpose(1, 2).requires_grad_(True) for _ in range(2))
+    do = torch.randn(2, 7, 4, 6, dtype=torch.float64)
+    with Products():
+        o, _ = hf_attention(m, q, k, v, None, scaling=0.4, softcap=5e3)
+        got = torch.autograd.grad(o, (q, k, v), do)
+    assert len(seen) == 6 and all(seen), seen
+    want = _capped64(q, k, v, 0.4, 5e3)
+    assert torch.allclose(o, want, atol=1e-6)  # (the probabilities are taken in fp32)
+    for a, b in zip(got, torch.autograd.grad(want, (q, k, v), do)):
+        assert torch.allclose(a, b, atol=1e-5)
