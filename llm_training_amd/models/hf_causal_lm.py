@@ -9,12 +9,11 @@ The model body runs through transformers; its attention is routed to our gfx950 
 ``llmt_hip``: the packed segment ids travel as a forward kwarg down to every attention call, so
 packed rows take the varlen kernel instead of a dense [B, 1, S, S] mask — the reference reaches the
 same end by patching ``_get_unpad_data`` for FA2 (hf_causal_lm.py:19-20). Calls the kernel cannot
-serve (head dims other than 64/96/128, non-causal modules, logit soft-capping with dropout or against a
-cache) run transformers' SDPA with the equivalent dense mask; soft-capping alone and attention dropout alone run in
-the kernels. The loss heads use our
-fused lm_head + cross-entropy on the final hidden states, and the ZeRO engine shards the HF model by
-its ``_no_split_modules`` blocks. ``hf_config`` builds a random-init model from a config dict (no
-checkpoint needed); ``hf_path`` loads a LOCAL checkpoint.
+serve (head dims other than 64/96/128, non-causal modules, logit soft-capping with dropout, against a cache or in
+fp16 / fp32 on the GPU) run transformers' SDPA with the equivalent dense mask; soft-capping alone and attention dropout
+alone run in the kernels. The loss heads use our fused lm_head + cross-entropy on the final hidden states, and the
+ZeRO engine shards the HF model by its ``_no_split_modules`` blocks. ``hf_config`` builds a random-init model from a
+config dict (no checkpoint needed); ``hf_path`` loads a LOCAL checkpoint.
 """
 from __future__ import annotations
 
@@ -75,6 +74,8 @@ def hf_attention(module, query, key, value, attention_mask, scaling=None, dropou
     why = None
     if softcap is not None and (dropout or query.shape[2] != key.shape[2] or not 0.0 < softcap <= MAX_SOFTCAP):
         why = "logit soft-capping with dropout, against a cache or above the kernels' range"
+    elif softcap is not None and query.is_cuda and query.dtype != torch.bfloat16:
+        why = f"logit soft-capping in {query.dtype}"  # (flash_attention would hold the scores in fp32)
     elif D not in (64, 96, 128) and query.is_cuda:
         why = f"head dim {D}"
     elif not getattr(module, "is_causal", True) or attention_mask is not None:

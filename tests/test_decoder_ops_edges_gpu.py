@@ -1,8 +1,12 @@
 """Calls of the decoder operators at the edge of what their documentation allows, on the GPU."""
+from types import SimpleNamespace
+
 import pytest
 import torch
 
 from llm_training_amd import ops
+from llm_training_amd.models.hf_causal_lm import hf_attention
+from llm_training_amd.ops import fused
 from test_attention_mod_gpu import MODS, compare, oracle
 from test_attention_mod_gpu import run as attention
 
@@ -78,3 +82,27 @@ def test_capped_scores_at_both_ends_and_values_of_any_size(D, softcap, size):
         compare(got, want, lim)
         plain = ops.flash_attention(q, k, v, softcap=softcap)
     assert plain.isfinite().all() and torch.equal(o == 0, plain == 0)
+
+
+@pytest.mark.parametrize("dtype,eps", [(torch.float16, 2.0 ** -11), (torch.float32, 2.0 ** -24)])
+def test_capped_attention_of_other_types_keeps_the_dense_path(dtype, eps, monkeypatch):
+    """fp16 / fp32 layers of a capped model hold the scores in their own type: flash_attention's torch form would take
+    twice the memory for fp16."""
+    monkeypatch.setattr(fused, "flash_attention", None)
+    torch.manual_seed(6)
+    B, H, S, D, cap, scale = 2, 4, 90, 64, 20.0, 0.125
+    q, k, v = (torch.randn(B, h, S, D, device=DEV).to(dtype) for h in (H, 2, 2))
+    m = SimpleNamespace(is_causal=True, training=False)
+    o, _ = hf_attention(m, q, k, v, None, scaling=scale, softcap=cap)
+    assert o.dtype == dtype
+    kd, vd = k.double().repeat_interleave(2, 1), v.double().repeat_interleave(2, 1)
+    i = torch.arange(S, device=DEV)
+    x = torch.matmul(q.double(), kd.transpose(-1, -2).contiguous()) * scale
+    s = (cap * torch.tanh(x / cap)).masked_fill(i[None] > i[:, None], float("-inf"))
+    p = torch.softmax(s, -1)
+    # scores: product, scale, quotient, tanh and cap rounded to the type, each half a step of at most |x|, beside fp32 sums
+    # over D; a score off by t changes p by a factor of up to 1 +- 2 t; p and the output are rounded once each
+    mag = torch.matmul(q.double().abs(), kd.abs().transpose(-1, -2).contiguous()).max() * scale
+    t = 5 * eps * x.abs().max() + (D + 1) * 2.0 ** -24 * mag
+    lim = (2.5 * t + 2 * eps + S * 2.0 ** -24) * torch.matmul(p, vd.abs()).transpose(1, 2) + 2.0 ** -24
+    assert ((o.double() - torch.matmul(p, vd).transpose(1, 2)).abs() <= lim).all()
