@@ -89,3 +89,15 @@ def test_dense_capped_attention_multiplies_by_contiguous_operands():
     assert torch.allclose(o, want, atol=1e-6)  # (the probabilities are taken in fp32)
     for a, b in zip(got, torch.autograd.grad(want, (q, k, v), do)):
         assert torch.allclose(a, b, atol=1e-5)
+
+
+def test_dense_attention_keeps_a_window_without_segments():
+    """A sliding window narrower than the sequence, no segment ids: capped (a cap beyond the kernels' range)."""
+    m = SimpleNamespace(is_causal=True, training=False)
+    torch.manual_seed(1)
+    q = torch.randn(2, 4, 9, 6)
+    k, v = (torch.randn(2, 2, 9, 6) for _ in range(2))
+    for window in (1, 4, 8, 9, 30):
+        o, _ = hf_attention(m, q, k, v, None, scaling=0.4, softcap=5e3, sliding_window=window)
+        want = _capped64(q.double(), k.double(), v.double(), 0.4, 5e3, window)
+        assert torch.allclose(o.double(), want, atol=1e-5), window  # (fp32: some dozen roundings of values up to 4)
