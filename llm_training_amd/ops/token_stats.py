@@ -64,6 +64,8 @@ class _LinearTokenStatsFn(Function):
         need_h, need_w = ctx.needs_input_grad[:2]
         dh = torch.empty_like(h) if need_h else None
         dw = dw_accumulator(w, N, chunk) if need_w else None
+        if need_w and N == 0:  # (no chunk writes it)
+            dw.zero_()
         wt = weight_t(w, N) if need_h and N > chunk else None
         for s0 in range(0, N, chunk):
             s = slice(s0, min(N, s0 + chunk))

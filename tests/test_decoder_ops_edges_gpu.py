@@ -106,3 +106,23 @@ def test_capped_attention_of_other_types_keeps_the_dense_path(dtype, eps, monkey
     t = 5 * eps * x.abs().max() + (D + 1) * 2.0 ** -24 * mag
     lim = (2.5 * t + 2 * eps + S * 2.0 ** -24) * torch.matmul(p, vd.abs()).transpose(1, 2) + 2.0 ** -24
     assert ((o.double() - torch.matmul(p, vd).transpose(1, 2)).abs() <= lim).all()
+
+
+@pytest.mark.parametrize("buffer", [None, torch.bfloat16, torch.float32])
+def test_linear_token_stats_of_no_rows(buffer):
+    """No rows: the weight's gradient is zero (nothing is added to a buffer), whatever its memory held."""
+    w = torch.randn(96, 64, device=DEV).bfloat16().requires_grad_(True)
+    h = torch.randn(0, 64, device=DEV).bfloat16().requires_grad_(True)
+    labels = torch.zeros(0, device=DEV, dtype=torch.long)
+    junk = [torch.full(w.shape, 7.0, device=DEV, dtype=t) for t in (torch.bfloat16, torch.float32)]
+    del junk
+    if buffer is None:
+        r = ops.linear_token_stats(h, w, labels, top_k=2)
+        gh, gw = torch.autograd.grad(r.logps.sum() + r.entropy.sum(), (h, w))
+        assert gh.shape == (0, 64) and not gw.any()
+        return
+    w.main_grad = torch.full(w.shape, 3.0, device=DEV, dtype=buffer)
+    for added, value in ((True, 3.0), (False, 0.0)):
+        w.grad_added = added
+        ops.linear_token_stats(h, w, labels).logps.sum().backward()
+        assert (w.main_grad == value).all() and w.grad_added
