@@ -38,7 +38,8 @@ class _EmbeddingFn(Function):
         if not ctx.needs_input_grad[1]:
             return None, None, None, None, None, None
         mg = getattr(w, "main_grad", None)
-        if on_kernels(g):
+        # (a backward that is differentiated itself, create_graph=True, takes the torch form below)
+        if on_kernels(g) and not (mg is None and torch.is_grad_enabled() and g.requires_grad):
             fresh = mg is None
             dw = torch.empty(ctx.wshape, dtype=w.dtype, device=g.device) if fresh else mg.view(ctx.wshape)
             lib().embedding_bwd_(ids.contiguous(), g.contiguous(), dw, v0, min(v1 - v0, ctx.wshape[0]), scale,

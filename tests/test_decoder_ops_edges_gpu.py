@@ -7,6 +7,7 @@ import torch
 from llm_training_amd import ops
 from llm_training_amd.models.hf_causal_lm import hf_attention
 from llm_training_amd.ops import fused
+from llm_training_amd.ops.embedding import vocab_embedding
 from test_attention_mod_gpu import MODS, compare, oracle
 from test_attention_mod_gpu import run as attention
 
@@ -126,3 +127,16 @@ def test_linear_token_stats_of_no_rows(buffer):
         w.grad_added = added
         ops.linear_token_stats(h, w, labels).logps.sum().backward()
         assert (w.main_grad == value).all() and w.grad_added
+
+
+def test_embedding_of_a_model_keeps_its_second_derivative():
+    """Linear in the table: the gradient is differentiable in dY, as it was in front of the kernels."""
+    torch.manual_seed(7)
+    w = torch.randn(9, 8, device=DEV).requires_grad_(True)
+    g = torch.randn(5, 8, device=DEV).requires_grad_(True)
+    ids = torch.tensor([1, 1, 2, 8, 1], device=DEV)
+    dw, = torch.autograd.grad(vocab_embedding(ids, w, 0, 9, False, 0.5), w, g, create_graph=True)
+    dg, = torch.autograd.grad(dw.square().sum(), g)
+    # (three summands at most and a factor that is a power of two: a few roundings of values up to 8)
+    assert torch.allclose(dw.detach(), torch.zeros_like(w).index_add(0, ids, 0.5 * g.detach()), atol=1e-5)
+    assert torch.allclose(dg, 2 * 0.5 * dw.detach()[ids], atol=1e-5)
