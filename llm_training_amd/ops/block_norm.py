@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import torch
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from . import reference as ref
 from .native import lib, on_kernels
@@ -41,6 +42,7 @@ class _NormAddNormFn(Function):
         return (s,) if w2 is None else (h, s)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, *grads):
         x, res, r1, r2 = ctx.saved_tensors
         w1, w2, gate = ctx.w
@@ -86,6 +88,7 @@ class _RefNormAddNormFn(Function):
         return (s,) if w2 is None else (h, s)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, *grads):
         from .fused import _wgrad_vec
         x, res = ctx.saved_tensors

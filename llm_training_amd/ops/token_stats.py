@@ -9,6 +9,7 @@ from typing import NamedTuple
 
 import torch
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from . import reference as ref
 from .native import lib, on_kernels, use_native
@@ -51,6 +52,7 @@ class _LinearTokenStatsFn(Function):
         return logps, ent, top, ids
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, g_logp, g_ent, g_top, _):
         from .fused import _apply_weight_grad, dw_accumulator, dw_add_chunk, mm_nn, mm_nt, weight_t
         h, labels, norm, ent, ids = ctx.saved_tensors

@@ -1,6 +1,7 @@
 """Calls of the decoder operators at the edge of what their documentation allows, as far as the host decides them."""
 from types import SimpleNamespace
 
+import pytest
 import torch
 from torch.utils._python_dispatch import TorchDispatchMode
 
@@ -101,3 +102,12 @@ def test_dense_attention_keeps_a_window_without_segments():
         o, _ = hf_attention(m, q, k, v, None, scaling=0.4, softcap=5e3, sliding_window=window)
         want = _capped64(q.double(), k.double(), v.double(), 0.4, 5e3, window)
         assert torch.allclose(o.double(), want, atol=1e-5), window  # (fp32: some dozen roundings of values up to 4)
+
+
+def test_norm_add_norm_refuses_a_second_derivative():
+    """Its backward has no graph: differentiating it says so instead of leaving terms out."""
+    x, res, w = torch.randn(3, 8).requires_grad_(True), torch.randn(3, 8), torch.rand(8)
+    _, s = ops.norm_add_norm(x, res, w, None, 1e-5)
+    g, = torch.autograd.grad(s.square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.square().sum().backward()

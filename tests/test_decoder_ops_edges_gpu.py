@@ -140,3 +140,18 @@ def test_embedding_of_a_model_keeps_its_second_derivative():
     # (three summands at most and a factor that is a power of two: a few roundings of values up to 8)
     assert torch.allclose(dw.detach(), torch.zeros_like(w).index_add(0, ids, 0.5 * g.detach()), atol=1e-5)
     assert torch.allclose(dg, 2 * 0.5 * dw.detach()[ids], atol=1e-5)
+
+
+def test_second_derivatives_of_the_python_nodes_are_refused():
+    """The nodes for gradient buffers and the linear head's say so instead of leaving terms out."""
+    x = torch.randn(4, 8, device=DEV).requires_grad_(True)
+    v = torch.rand(8, device=DEV).requires_grad_(True)
+    v.main_grad = torch.zeros(8, device=DEV)
+    h = torch.randn(4, 64, device=DEV).bfloat16().requires_grad_(True)
+    t = torch.randn(96, 64, device=DEV).bfloat16()
+    labels = torch.zeros(4, dtype=torch.long, device=DEV)
+    for y, z in ((ops.norm_add_norm(x, x.detach(), v, None, 1e-6)[1], x),
+                 (ops.linear_token_stats(h, t, labels).logps, h)):
+        d, = torch.autograd.grad(y.float().square().sum(), z, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            d.float().square().sum().backward()
