@@ -11,6 +11,11 @@ from torch.autograd import Function
 from .native import lib, on_kernels
 
 
+def _rows(v0, v1, shape):
+    """Rows of the table that hold ids (a shard wholly behind a small vocabulary has none: v1 < v0)."""
+    return max(0, min(v1 - v0, shape[0]))
+
+
 class _EmbeddingFn(Function):
     @staticmethod
     def forward(ctx, ids, w, v0, v1, sharded, scale):
@@ -19,7 +24,7 @@ class _EmbeddingFn(Function):
         ctx.wshape = w.shape
         ctx.cfg = (v0, v1, sharded, scale)
         if on_kernels(w):
-            return lib().embedding_fwd(ids.contiguous(), w.contiguous(), v0, min(v1 - v0, w.shape[0]), scale, sharded)
+            return lib().embedding_fwd(ids.contiguous(), w.contiguous(), v0, _rows(v0, v1, w.shape), scale, sharded)
         local = ids - v0
         if sharded:  # vocab-sharded: rows owned by other ranks contribute zeros
             mask = (ids >= v0) & (ids < v1)
@@ -42,7 +47,7 @@ class _EmbeddingFn(Function):
         if on_kernels(g) and not (mg is None and torch.is_grad_enabled() and g.requires_grad):
             fresh = mg is None
             dw = torch.empty(ctx.wshape, dtype=w.dtype, device=g.device) if fresh else mg.view(ctx.wshape)
-            lib().embedding_bwd_(ids.contiguous(), g.contiguous(), dw, v0, min(v1 - v0, ctx.wshape[0]), scale,
+            lib().embedding_bwd_(ids.contiguous(), g.contiguous(), dw, v0, _rows(v0, v1, ctx.wshape), scale,
                                  not fresh and bool(getattr(w, "grad_added", False)), sharded)
             if fresh:
                 return None, dw, None, None, None, None

@@ -155,3 +155,13 @@ def test_second_derivatives_of_the_python_nodes_are_refused():
         d, = torch.autograd.grad(y.float().square().sum(), z, create_graph=True)
         with pytest.raises(RuntimeError, match="once_differentiable"):
             d.float().square().sum().backward()
+
+
+@pytest.mark.parametrize("N", [5, 700])
+def test_embedding_shard_behind_the_vocabulary(N):
+    """A vocabulary smaller than the shards' rows: the last ranks' shards begin behind it and hold nothing."""
+    w = torch.randn(2, 8, device=DEV).requires_grad_(True)
+    ids = torch.arange(N, device=DEV) % 10
+    y = vocab_embedding(ids, w, 12, 10, True)
+    assert y.shape == (N, 8) and not y.any()
+    assert not torch.autograd.grad(y, w, torch.ones_like(y))[0].any()
