@@ -91,7 +91,8 @@ def hf_attention(module, query, key, value, attention_mask, scaling=None, dropou
         logger.warning("HFCausalLM attention: %s is not served by the HIP flash kernel; using SDPA", why)
     from transformers.integrations.sdpa_attention import sdpa_attention_forward
     Sq, Sk = query.shape[2], key.shape[2]
-    if attention_mask is None and seg is None and sliding_window is not None and sliding_window < Sk == Sq:
+    causal = getattr(module, "is_causal", True)
+    if attention_mask is None and seg is None and causal and sliding_window is not None and sliding_window < Sk == Sq:
         seg = torch.zeros(query.shape[0], Sk, dtype=torch.int32)  # one sequence: the mask is the window's
     if attention_mask is None and seg is not None:
         attention_mask = _dense_mask(seg.to(query.device), query.shape[2], query.dtype, sliding_window)

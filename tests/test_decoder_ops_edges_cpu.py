@@ -111,3 +111,13 @@ def test_norm_add_norm_refuses_a_second_derivative():
     g, = torch.autograd.grad(s.square().sum(), x, create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         g.square().sum().backward()
+
+
+def test_dense_attention_of_a_module_without_a_causal_mask():
+    """No causal mask comes with the window there: SDPA over all keys, as without one."""
+    m = SimpleNamespace(is_causal=False, training=False)
+    torch.manual_seed(2)
+    q, k, v = (torch.randn(1, 2, 6, 8) for _ in range(3))
+    o, _ = hf_attention(m, q, k, v, None, scaling=0.3, sliding_window=2)
+    want = torch.softmax(q @ k.transpose(-1, -2) * 0.3, -1) @ v
+    assert torch.allclose(o, want.transpose(1, 2), atol=1e-5)
