@@ -48,16 +48,14 @@ class _BatchProduct(torch.autograd.Function):
     library's batched bf16 products have faulted on right operands that are transposed views."""
 
     @staticmethod
-    @torch.amp.custom_fwd(device_type="cuda")
     def forward(ctx, a, b, trans):
         ctx.save_for_backward(a, b)
         ctx.trans = trans
         return torch.matmul(a, (b.transpose(-1, -2) if trans else b).contiguous())
 
     @staticmethod
-    @torch.amp.custom_bwd(device_type="cuda")
     def backward(ctx, g):
-        a, b = ctx.saved_tensors
+        a, b = (t.to(g.dtype) for t in ctx.saved_tensors)  # (under autocast the product's type is not theirs)
         if ctx.trans:
             return torch.matmul(g, b.contiguous()), torch.matmul(g.transpose(-1, -2), a.contiguous()), None
         return (torch.matmul(g, b.transpose(-1, -2).contiguous()),

@@ -121,3 +121,17 @@ def test_dense_attention_of_a_module_without_a_causal_mask():
     o, _ = hf_attention(m, q, k, v, None, scaling=0.3, sliding_window=2)
     want = torch.softmax(q @ k.transpose(-1, -2) * 0.3, -1) @ v
     assert torch.allclose(o, want.transpose(1, 2), atol=1e-5)
+
+
+def test_dense_capped_attention_under_autocast():
+    """fp32 tensors, products in bf16: the gradients come back in fp32, as near as bf16 operands leave them."""
+    m = SimpleNamespace(is_causal=True, training=False)
+    torch.manual_seed(3)
+    q, k, v = (torch.randn(1, 2, 6, 8).requires_grad_(True) for _ in range(3))
+    with torch.autocast("cpu", dtype=torch.bfloat16):
+        o, _ = hf_attention(m, q, k, v, None, scaling=0.3, softcap=5e3)
+    got = torch.autograd.grad(o.float().sum(), (q, k, v))
+    want = torch.autograd.grad(_capped64(*(t.double() for t in (q, k, v)), 0.3, 5e3).sum(), (q, k, v))
+    for a, b in zip(got, want):
+        # a dozen bf16 roundings on the way, 2^-8 each of values up to 4, in sums of up to 8
+        assert a.dtype == torch.float32 and (a - b).abs().max() < 12 * 2.0 ** -8 * 4 * 8 ** 0.5
