@@ -169,7 +169,7 @@ __global__ __launch_bounds__(64) void embed_scan_kernel(int* __restrict__ hist, 
   h[(int64_t)nblk * kRadix] = sum;
 }
 
-// step 3: stable scatter by the digit at `shift`. Each wave owns 512 consecutive keys of the tile and takes them in
+// step 3: stable scatter by the digit at `shift`. Each wave owns 256 consecutive keys of the tile and takes them in
 // rounds of 64: the lanes with an equal digit find each other through one ballot per bit, so a lane's place is the
 // wave's running count of its digit plus the equal lanes below it.
 template <typename I, bool FIRST>

@@ -46,8 +46,8 @@ using namespace llmt;
 // pairs, the un-pipelined dK/dV loop, the separate prep pass) were removed after their A/Bs
 // (profiles/r5_attention_fwd4.md, r5_dkdv6.md, r3_attention_head_pairs_ab.jsonl, r4_negative_probes.jsonl).
 // Knobs, read per launch (recorded by ops/native.py llmt_env() into run metadata):
-//   LLMT_FA_GENERIC=1     the generic kernels for every launch (numerics reference);
-//   LLMT_FA_RANGE_MASK=0  per-element mask compares instead of range masks (A/B reference);
+//   LLMT_FA_GENERIC=1     the generic kernels for every launch on plain scores (numerics reference);
+//   LLMT_FA_RANGE_MASK=0  per-element mask compares instead of range masks, plain scores only (A/B reference);
 //   LLMT_FA_EARLY_DMA=0   row loads before the first ring tiles in the prologues (A/B reference);
 //   LLMT_FA_BMAJOR=0      batch-interleaved block order of dense rows (A/B reference; B4 S8192 Hq32 Hkv8 with
 //                         the default batch-major order: forward 2.102 -> 2.068 ms, backward 7.795 -> 7.732 ms).

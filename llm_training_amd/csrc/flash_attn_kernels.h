@@ -246,7 +246,8 @@ struct AttnArgs {
 // end are visible to every query of the document. Kernel template argument MOD: the sum of
 //   kModCap   with r = 1 / (1 + exp2(cap_k x)), tanh = 1 - 2 r: one exp2, one reciprocal and two adds per score
 //             instead of a tanh; its derivative is 4 (r - r^2), whose 4 goes into the gradients' final scale;
-//   kModBias  one subtraction and one FMA per score (|.| is an operand modifier);
+//   kModBias  forward: an addition per score (the row's part and an element's constant ride in other instructions, see
+//             there); backward: one subtraction and one FMA per score (|.| is an operand modifier);
 //   kModPre   kernels without either that read a.pend. (Every MOD kernel reads it: a prefix only changes the index
 //             ranges of the masks and the tiles walked, nothing per score.) As the kernels on plain scores they take
 //             maxima and masks of raw products, so a scale <= 0 runs the kernels with a bias, of slope 0.

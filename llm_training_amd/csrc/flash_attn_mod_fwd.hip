@@ -7,7 +7,7 @@ hipError_t launch_mod_fwd(const AttnArgs& a, int D, int mod, unsigned grid, hipS
 #define LLMT_MOD(DD, M)                                                       \
   if (M == kModCap || a.olo)                                                  \
     fa_fwd3_kernel<DD, 2, 1, 4, false, true, M><<<grid, 256, 0, stream>>>(a); \
-  else                                                                        \
+  else /* (kModCap has no such form: it is not instantiated a second time) */ \
     fa_fwd3_kernel<DD, 2, 1, 4, false, M == kModCap, M><<<grid, 256, 0, stream>>>(a)
   LLMT_MOD_KERNELS(LLMT_MOD)
 #undef LLMT_MOD

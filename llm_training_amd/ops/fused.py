@@ -1002,7 +1002,9 @@ def flash_attention(q, k, v, causal: bool = True, segment_ids=None, window: int 
     ``alibi_slopes`` [Hq] (no gradient) then subtracts slope_h |i - j| from the score of query i and key j;
     ``prefix_mask`` [B, S] marks tokens at the head of documents that all tokens of the document see, also the
     ones in front of them (causal attention otherwise; a window still bounds the distance backwards), or
-    ``prefix_ends``: its precomputed :func:`prefix_ends`."""
+    ``prefix_ends``: its precomputed :func:`prefix_ends`. ``scale`` may be of any sign with them. The kernels' forward
+    that a gradient follows normalises by the sum of the rounded probabilities; without one, a bias, a prefix or a cap
+    above 60 by that of the unrounded ones: O may then differ in its last bit."""
     mod = _score_mod(q, causal, segment_ids, dropout_p, softcap, alibi_slopes, prefix_mask, prefix_ends)
     scale = scale if scale is not None else 1.0 / math.sqrt(q.shape[-1])
     if mod is not None:

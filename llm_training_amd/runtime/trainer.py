@@ -284,7 +284,7 @@ class Trainer:
         self.pc = ParallelContext.create(st.data_parallel_size, st.tensor_parallel_size, device)
         seed = self.seed if self.seed is not None else 42
         if self.deterministic:
-            # bitwise-reproducible steps: sort-based embedding backward (models/modules.py); every HIP
+            # bitwise-reproducible steps: the embedding's gradient sums sorted tokens (ops/embedding.py); every HIP
             # kernel already reduces in a fixed order (no float atomics in the backward)
             torch.use_deterministic_algorithms(True, warn_only=True)
             os.environ["LLMT_DETERMINISTIC"] = "1"
